@@ -6,7 +6,6 @@ Each operator has its form for prompts and, where it keeps a state, its form for
 ``run`` computes the plain form in elementary torch operations, or calls the framework's
 kernels where ``own`` is true; ``exact`` restates the definitions in 64 bits.
 """
-import functools
 import math
 import os
 import sys
@@ -323,9 +322,7 @@ def _plain_norm(s):
     return out
 
 
-@functools.lru_cache(maxsize=None)
 def _framework():
-    """The package, imported once, as a program does."""
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                         "pto-fuser_b200")
     if root not in sys.path:
