@@ -11,9 +11,9 @@
 // least: one block of 1024 threads took 121 us for 4096 x 16384 bf16, two of 512 take 80.
 //
 // bf16 with a residual, us and share of the copy bandwidth: 16384 x 8192 to e4m3 with a scale
-// for 128 columns 143 (1.0), 4096 x 16384 80 (1.0). Rows that begin on no 16 bytes:
+// for 128 columns 148, 4096 x 16384 80 (1.0). Rows that begin on no 16 bytes:
 // 3001 x 5003 f16 with an fp32 residual 31 (0.90; 45 element by element). Such rows to e4m3
-// with a scale a group go element by element, bound by instructions: 4096 x 5001 takes 53
+// with a scale a group go element by element, bound by instructions: 4096 x 5001 takes 54
 // where 5000 columns take 35.
 #include <cuda_fp8.h>
 
@@ -53,9 +53,39 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// amax / 448 by a product with the rounded reciprocal, which is off by one more half unit
-__device__ __forceinline__ float scale_of(float amax) {
-  return max_nan(amax * (1.f / kFp8Max), kTinyScale);
+// Quotients rounded once, as the definition has them: products with rounded reciprocals give 59 %
+// of the scales another last bit, and eight of a million codes the neighbouring e4m3 value.
+// With r within a unit in the last place of 1 / s, q = y r is off by two units at most, and
+// adding r times the remainder y - q s of a fused product rounds to y / s (P. Markstein,
+// Computation of elementary functions on the IBM RISC System/6000 processor, 1990), or, with r
+// not correctly rounded, to its neighbour where y / s lies within 2^-22 units of the middle
+// between two values. That is two instructions a value more than the product alone:
+// 16384 x 8192 to e4m3 with a scale for 128 columns takes 148 us, with products 144, with the
+// library's division and reciprocal 158.
+constexpr float kLargest = 3.40282347e38f;  // largest finite fp32 value
+
+// Scale and quotients of the values whose largest magnitude is amax.
+struct Scale {
+  float s, r, minus_s;
+  // y / s. An infinite scale has no remainder: 0 for finite y. A quotient of zero is +0.
+  __device__ __forceinline__ float quotient(float y) const {
+    const float q = y * r;
+    return fmaf(fmaf(q, minus_s, y), r, q);
+  }
+  __device__ __forceinline__ float2 quotient(f32x2 y) const {
+    const f32x2 r2 = pack2(r, r), q = mul2(y, r2);
+    return unpack2(fma2(fma2(q, pack2(minus_s, minus_s), y), r2, q));
+  }
+};
+__device__ __forceinline__ Scale scale_of(float amax) {
+  constexpr float r = 1.f / kFp8Max;
+  const bool finite = amax <= kLargest;
+  const float q = amax * r, rest = finite ? fmaf(q, -kFp8Max, amax) : 0.f;
+  Scale o;
+  o.s = max_nan(fmaf(rest, r, q), kTinyScale);
+  o.r = fast_rcp(o.s);  // s is a normal number, its reciprocal at most 2^126
+  o.minus_s = finite ? -o.s : 0.f;
+  return o;
 }
 
 // Sum (MAX = false) or NaN-keeping maximum over the TPR threads of a row, on every thread.
@@ -189,11 +219,10 @@ __global__ void __launch_bounds__(threads_of(TPR), TPR > 512 ? 1 : TPR > 256 ? 2
     }
     return;
   }
-  float s = 0.f, inv = 0.f;
+  Scale by;
   if (QUANT == kQuantRow) {
-    s = scale_of(row_reduce<TPR, true>(amax, red));
-    inv = fast_rcp(s);  // s is a normal number, its reciprocal at most 2^126
-    if (live && tx == 0) a.scale[row] = s;
+    by = scale_of(row_reduce<TPR, true>(amax, red));
+    if (live && tx == 0) a.scale[row] = by.s;
   }
   const int seg = a.group / VEC;  // threads of a group, a power of two up to a warp
   uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.y_rs;
@@ -210,16 +239,14 @@ __global__ void __launch_bounds__(threads_of(TPR), TPR > 512 ? 1 : TPR > 256 ? 2
 #pragma unroll
       for (int off = 1; off < 32; off *= 2)
         if (off < seg) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, off));
-      s = scale_of(m);
-      inv = fast_rcp(s);
-      if (live && c < a.D && tx % seg == 0) a.scale[row * a.groups + (c >> a.shift)] = s;
+      by = scale_of(m);
+      if (live && c < a.D && tx % seg == 0) a.scale[row * a.groups + (c >> a.shift)] = by.s;
     }
     if (live && c < a.D) {
       Pack<uint16_t, VEC / 2> o;
 #pragma unroll
       for (int k = 0; k < VEC / 2; ++k)
-        o.v[k] = __nv_cvt_float2_to_fp8x2(unpack2(mul2(h[i][k], pack2(inv, inv))), __NV_SATFINITE,
-                                          __NV_E4M3);
+        o.v[k] = __nv_cvt_float2_to_fp8x2(by.quotient(h[i][k]), __NV_SATFINITE, __NV_E4M3);
       st_pack<uint16_t, VEC / 2>(reinterpret_cast<uint16_t*>(y + c), o);
     }
   }
@@ -313,11 +340,10 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of(TPR, 4 * NV)) rms_n
       }
     }
   }
-  float inv = 1.f;
+  Scale by;
   if (QUANT == kQuantRow) {
-    const float s = scale_of(row_reduce<TPR, true>(amax, red));
-    inv = fast_rcp(s);
-    if (live && tx == 0) a.scale[row] = s;
+    by = scale_of(row_reduce<TPR, true>(amax, red));
+    if (live && tx == 0) a.scale[row] = by.s;
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -339,7 +365,7 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of(TPR, 4 * NV)) rms_n
       Pack<uint16_t, 2> o;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        o.v[k] = __nv_cvt_float2_to_fp8x2(unpack2(mul2(h[i][k], pack2(inv, inv))), __NV_SATFINITE, __NV_E4M3);
+        o.v[k] = __nv_cvt_float2_to_fp8x2(by.quotient(h[i][k]), __NV_SATFINITE, __NV_E4M3);
       if (whole(c)) {
         st_pack<uint16_t, 2>(reinterpret_cast<uint16_t*>(y + c), o);
       } else {
@@ -392,7 +418,7 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of(TPR, 4 * NSEG)) rms
   ss = row_reduce<TPR, false>(ss, red);
   const float r = rsqrtf(fmaf(ss, a.inv_d, a.eps));
   auto y_of = [&](int c, float v) { return c < a.D ? v * r * ld_beta_any(a.w, a.w_dtype, c) : 0.f; };
-  float s = 0.f;
+  Scale by;
   if (QUANT == kQuantRow) {
     float amax = 0.f;
     each([&](int c, int i) {
@@ -400,16 +426,17 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of(TPR, 4 * NSEG)) rms
 #pragma unroll
       for (int k = 0; k < 4; ++k) amax = max_nan(amax, fabsf(y_of(c + 32 * k, h[i][k])));
     });
-    s = scale_of(row_reduce<TPR, true>(amax, red));
-    if (live && threadIdx.x % TPR == 0) a.scale[row] = s;
+    by = scale_of(row_reduce<TPR, true>(amax, red));
+    if (live && threadIdx.x % TPR == 0) a.scale[row] = by.s;
   }
   each([&](int c, int i) {
     if (!NSEG) load(c, h[i]);
-    float o[4], inv[4];
+    float o[4];
+    Scale of[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       o[k] = y_of(c + 32 * k, h[i][k]);
-      inv[k] = QUANT == kQuantRow ? fast_rcp(s) : 1.f;
+      of[k] = by;
     }
     if (QUANT == kQuantGroup) {
       // the bits of numbers without a sign are in their order, with NaN above all
@@ -430,10 +457,10 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of(TPR, 4 * NSEG)) rms
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float sk = scale_of(m[k]);
-        inv[k] = fast_rcp(sk);
+        if (k == 0 || a.group == 32 || (k == 2 && a.group == 64)) by = scale_of(m[k]);
+        of[k] = by;
         const int ck = c + 32 * k;
-        if (ck < D && (ck & (a.group - 1)) == 0) a.scale[row * a.groups + (ck >> a.shift)] = sk;
+        if (ck < D && (ck & (a.group - 1)) == 0) a.scale[row * a.groups + (ck >> a.shift)] = by.s;
       }
     }
 #pragma unroll
@@ -443,7 +470,7 @@ __global__ void __launch_bounds__(threads_of(TPR), blocks_of(TPR, 4 * NSEG)) rms
         if (RES) static_cast<TR*>(a.sum)[row * a.sum_rs + ck] = from_f32<TR>(h[i][k]);
         if (QUANT == kNoQuant) static_cast<T*>(a.y)[row * a.y_rs + ck] = from_f32<T>(o[k]);
         else static_cast<uint8_t*>(a.y)[row * a.y_rs + ck] =
-                 __nv_cvt_float_to_fp8(o[k] * inv[k], __NV_SATFINITE, __NV_E4M3);
+                 __nv_cvt_float_to_fp8(of[k].quotient(o[k]), __NV_SATFINITE, __NV_E4M3);
       }
     }
   });
