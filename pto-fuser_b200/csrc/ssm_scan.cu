@@ -260,7 +260,9 @@ __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const 
   }
   const f32x2 bias = a.bias ? pack2(a.bias[ca], a.bias[cz]) : pack2(0.f, 0.f);
   const f32x2 skip = a.D ? pack2(a.D[ca], a.D[cz]) : pack2(0.f, 0.f);
-  f32x2 dt_sum = pack2(0.f, 0.f);
+  // the chunk's sum of dt': what a tile adds goes into a compensated sum (W. Kahan, Further remarks
+  // on reducing truncation errors, 1965), so that its error does not grow with the chunk
+  f32x2 dt_tile = pack2(0.f, 0.f), dt_sum = dt_tile, dt_rest = dt_tile;
 
   const T* Bp = static_cast<const T*>(a.B) + b * a.B_bs + g * a.B_gs;
   const T* Cp = static_cast<const T*>(a.C) + b * a.C_bs + g * a.C_gs;
@@ -324,7 +326,7 @@ __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const 
     both.x = d;
     both.y = mul2(d, xv);
     if (t + TILE > t1 && t + g * TL + tok >= t1) both.x = both.y = pack2(0.f, 0.f);
-    if (SUMMARY && lane < TL) dt_sum = add2(dt_sum, both.x);
+    if (SUMMARY && lane < TL) dt_tile = add2(dt_tile, both.x);
     *reinterpret_cast<ulonglong2*>(sm.d[g % 2][tok * (CW / 2) + wp]) = both;
 #pragma unroll
     for (int i = 0; i < kBC; ++i) {
@@ -413,6 +415,13 @@ __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const 
       __syncwarp();  // the tile is free
     }
     if (t + 2 * TILE < t1) copy(t + 2 * TILE, st);
+    if (SUMMARY) {
+      const f32x2 more = add2(dt_tile, dt_rest), sum = add2(dt_sum, more);
+      const float2 rest = unpack2(add2(fma2(sum, pack2(-1.f, -1.f), dt_sum), more));
+      dt_rest = pack2(rest.x == rest.x ? rest.x : 0.f, rest.y == rest.y ? rest.y : 0.f);  // inf - inf
+      dt_sum = sum;
+      dt_tile = pack2(0.f, 0.f);
+    }
   }
 
   if (SUMMARY) {  // the lanes' parts of the sum of dt'

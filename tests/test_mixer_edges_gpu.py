@@ -61,3 +61,68 @@ def test_norm_to_8_bits_of_values_beyond_the_type():
             rest = torch.ones(D, dtype=torch.bool)
             rest[3] = False
             assert (y[:, rest][:, :100] == 0).all()
+
+
+# --------------------------------------------------------------------------- scan ----
+def _slots(N, T, D, n, dtype, packed=False, max_len=0):
+    """Chunk slots that a call's plan takes (0: whole sequences)."""
+    from pto_fuser import native as nv
+    p = nv.SsmScanParams(*[8] * 14, N, T, D, n, 1, nv.dtype_code(dtype), 1, packed, 0, max_len)
+    return nv.lib().ptof_ssm_scan_ws_bytes(ctypes.byref(p)) // (4 * D * (n + 1))
+
+
+@pytest.mark.parametrize("T,D,S", [(65536, 2048, 2048), (65536, 4096, 4096), (262144, 2048, 8192)])
+def test_scan_decay_over_long_chunks(T, D, S):
+    """Without inputs the state at a chunk's first token is exp(A sum dt') h0, from the chunks'
+    sums alone. Roundings, U = 2^-24 each: of a sum of 4 steps 3, of the compensated sum of
+    those 2, of its addition over lanes 2, of A log2(e) 2 and of its product with the sum 1, so
+    10 U of the exponent; 2^-22 for each exponential and U for each product."""
+    from pto_fuser import ssm_scan
+    assert _slots(1, T, D, 1, F32) == T // S
+    g = _gen(S)
+    dt = (0.5 + torch.rand(D, generator=g)) / S
+    A = -(0.3 + 0.4 * torch.rand(D, 1, generator=g))
+    zero, one = torch.zeros(1, 1, D).cuda(), torch.ones(1, 1, 1).cuda()
+    y, f = ssm_scan(zero.expand(1, T, D), dt.cuda().expand(1, T, D), A.cuda(), one.expand(1, T, 1),
+                    one.expand(1, T, 1), dt_softplus=False,
+                    initial_state=torch.ones(1, D, 1, device="cuda"))
+    j = np.arange(T // S)
+    arg = (j[:, None] * S + 1.0) * (_n64(dt) * _n64(A)[:, 0])
+    want = np.exp(arg)
+    tol = want * (np.abs(arg) * 10 * orc.U + (j[:, None] + 1) * (2.0 ** -22 + orc.U))
+    bad = ~(np.abs(_n64(y[0, ::S]) - want) <= tol)
+    assert not bad.any(), (int(bad.sum()), np.abs(_n64(y[0, ::S]) / want - 1).max())
+
+
+def _scan_inputs(T, D, n, dtype, seed=0):
+    g = _gen(seed)
+    r = lambda *s: torch.randn(*s, generator=g)
+    step = torch.exp(torch.rand(D, generator=g) * 4.6 - 9.2)
+    return dict(x=r(T, D).to(dtype), dt=(0.5 * r(T, D)).to(dtype), z=r(T, D).to(dtype),
+                A=-torch.arange(1, n + 1).float() * torch.exp(0.1 * r(D, n)),
+                B=r(T, 1, n).to(dtype), C=r(T, 1, n).to(dtype), D=1 + 0.1 * r(D),
+                bias=step + torch.log(-torch.expm1(-step)), init=r(1, D, n))
+
+
+@pytest.mark.parametrize("dtype,T,D,n,slots", [(BF16, 2100, 4096, 16, 0), (BF16, 16384, 4096, 16, 16),
+                                               (F16, 16384, 8192, 16, 8), (F32, 2000, 512, 16, 0),
+                                               (F16, 900, 40, 24, 0)])
+def test_scan_in_chunks_of_any_length_and_type(dtype, T, D, n, slots):
+    """Chunks of 1024 tokens and more, and shorter ones in 16-bit types, against the oracle over
+    a few of the channels (they do not meet)."""
+    from pto_fuser import ssm_scan
+    got = _slots(1, T, D, n, dtype)
+    assert got == slots if slots else got > 1
+    i = _scan_inputs(T, D, n, dtype, seed=T)
+    c = {k: v.cuda() for k, v in i.items()}
+    y, f = ssm_scan(c["x"][None], c["dt"][None], c["A"], c["B"][None], c["C"][None], D=c["D"],
+                    z=c["z"][None], dt_bias=c["bias"], initial_state=c["init"])
+    pick = torch.tensor([0, 1, D // 2 + 1, D - 1])
+    at = lambda k: _n64(i[k][..., pick])
+    ry, ty, rf, tf = orc.ssm_scan(at("x"), at("dt"), _n64(i["A"][pick]), _n64(i["B"]), _n64(i["C"]),
+                                  [(0, T)], D=at("D"), z=at("z"), dt_bias=at("bias"),
+                                  initial=_n64(i["init"][:, pick]))
+    gy, gf = _n64(y[0, :, pick]), _n64(f[:, pick])
+    eps, tiny = torch.finfo(dtype).eps, torch.finfo(dtype).tiny
+    assert (np.abs(gf - rf) <= tf + np.abs(rf) * orc.U).all()
+    assert (np.abs(gy - ry) <= ty + (np.abs(ry) + ty) * eps / 2 + tiny * eps / 2).all()
