@@ -17,6 +17,7 @@
 // of its dt' (the decay over a chunk is exp(A sum dt'), one exponential a state); the second
 // joins the records before its chunk and runs it from the right state.
 #include <cstring>
+#include <type_traits>
 
 #include "capi_internal.h"
 #include "mixer_ops.cuh"
@@ -347,65 +348,77 @@ __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const 
     if (t0 + TILE < t1) copy(t0 + TILE, 1);
     prepare(t0, 0, 0);
   }
-  int st = 0;
-  for (int t = t0; t < t1; t += TILE, st ^= 1) {
+  // One group of the tile at t: its recurrence and outputs, and the preparation of the next. With
+  // `guard` a state takes nothing from tokens behind the chunk, whose dt' x is zero but whose B,
+  // read as the last token's, may be infinite: zero times infinity would stay in it. Kept apart
+  // so that the tiles before the last go without a test inside.
+  auto group = [&](auto guard, int t, int st, int g) {
+    T* tx = &sm.tile[st][0][(g * TL + tok) * CW + 2 * wp];
+    f32x2 part[TL], xv, zv;
+    if (!SUMMARY) {
+      xv = pair_of(ld_pack<T, 2>(tx));
+      if (zp) zv = pair_of(ld_pack<T, 2>(tx + 2 * TILE * CW));
+    }
+#pragma unroll
+    for (int i0 = 0; i0 < TL; i0 += G) {
+      f32x2 E[G][SPL], X[G][SPL];
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const ulonglong2 both = *reinterpret_cast<const ulonglong2*>(sm.d[g % 2][(i0 + i) * (CW / 2) + wp]);
+        const float2 dx = unpack2(both.y);
+        const Pack<float, SPL> bv = ld_pack<float, SPL>(&sm.bc[g % 2][0][(i0 + i) * NP + lane * SPL]);
+#pragma unroll
+        for (int k = 0; k < SPL; ++k) {
+          const float2 u = unpack2(mul2(both.x, A2[k]));
+          E[i][k] = pack2(fast_exp2(u.x), fast_exp2(u.y));
+          X[i][k] = pack2(dx.x * bv.v[k], dx.y * bv.v[k]);
+          if (guard.value && t + g * TL + i0 + i >= t1) X[i][k] = pack2(0.f, 0.f);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+#pragma unroll
+        for (int k = 0; k < SPL; ++k) h[k] = E[i][k] = fma2(E[i][k], h[k], X[i][k]);
+      }
+      if (!SUMMARY) {
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          const Pack<float, SPL> cv = ld_pack<float, SPL>(&sm.bc[g % 2][1][(i0 + i) * NP + lane * SPL]);
+          float2 y2 = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < SPL; ++k) {
+            const float2 u = unpack2(E[i][k]);
+            y2.x = k ? fmaf(cv.v[k], u.x, y2.x) : cv.v[k] * u.x;
+            y2.y = k ? fmaf(cv.v[k], u.y, y2.y) : cv.v[k] * u.y;
+          }
+          part[i0 + i] = pack2(y2.x, y2.y);
+        }
+      }
+    }
+    if (g + 1 < NG) prepare(t, st, g + 1);
+    else prepare(t + TILE, st ^ 1, 0);  // (behind the last tile: of no use and not used)
+    if (!SUMMARY) {
+      f32x2 v = transpose_sum<TL>(part, tok);
+#pragma unroll
+      for (int off = TL; off < LANES; off *= 2)
+        v = add2(v, __shfl_xor_sync(0xffffffffu, v, off));
+      v = fma2(skip, xv, v);
+      if (zp) v = mul2(v, silu2(zv));
+      if (lane < TL) st_pair<T>(tx, v);  // over x, which all have read
+    }
+  };
+  auto tile = [&](auto guard, int t, int st) {
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       if (g == NG - 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncwarp();
-      T* tx = &sm.tile[st][0][(g * TL + tok) * CW + 2 * wp];
-      f32x2 part[TL], xv, zv;
-      if (!SUMMARY) {
-        xv = pair_of(ld_pack<T, 2>(tx));
-        if (zp) zv = pair_of(ld_pack<T, 2>(tx + 2 * TILE * CW));
-      }
-#pragma unroll
-      for (int i0 = 0; i0 < TL; i0 += G) {
-        f32x2 E[G][SPL], X[G][SPL];
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-          const ulonglong2 both = *reinterpret_cast<const ulonglong2*>(sm.d[g % 2][(i0 + i) * (CW / 2) + wp]);
-          const float2 dx = unpack2(both.y);
-          const Pack<float, SPL> bv = ld_pack<float, SPL>(&sm.bc[g % 2][0][(i0 + i) * NP + lane * SPL]);
-#pragma unroll
-          for (int k = 0; k < SPL; ++k) {
-            const float2 u = unpack2(mul2(both.x, A2[k]));
-            E[i][k] = pack2(fast_exp2(u.x), fast_exp2(u.y));
-            X[i][k] = pack2(dx.x * bv.v[k], dx.y * bv.v[k]);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-#pragma unroll
-          for (int k = 0; k < SPL; ++k) h[k] = E[i][k] = fma2(E[i][k], h[k], X[i][k]);
-        }
-        if (!SUMMARY) {
-#pragma unroll
-          for (int i = 0; i < G; ++i) {
-            const Pack<float, SPL> cv = ld_pack<float, SPL>(&sm.bc[g % 2][1][(i0 + i) * NP + lane * SPL]);
-            float2 y2 = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int k = 0; k < SPL; ++k) {
-              const float2 u = unpack2(E[i][k]);
-              y2.x = k ? fmaf(cv.v[k], u.x, y2.x) : cv.v[k] * u.x;
-              y2.y = k ? fmaf(cv.v[k], u.y, y2.y) : cv.v[k] * u.y;
-            }
-            part[i0 + i] = pack2(y2.x, y2.y);
-          }
-        }
-      }
-      if (g + 1 < NG) prepare(t, st, g + 1);
-      else prepare(t + TILE, st ^ 1, 0);  // (behind the last tile: of no use and not used)
-      if (!SUMMARY) {
-        f32x2 v = transpose_sum<TL>(part, tok);
-#pragma unroll
-        for (int off = TL; off < LANES; off *= 2)
-          v = add2(v, __shfl_xor_sync(0xffffffffu, v, off));
-        v = fma2(skip, xv, v);
-        if (zp) v = mul2(v, silu2(zv));
-        if (lane < TL) st_pair<T>(tx, v);  // over x, which all have read
-      }
+      group(guard, t, st, g);
     }
+  };
+  int st = 0;
+  for (int t = t0; t < t1; t += TILE, st ^= 1) {
+    if (t + TILE <= t1) tile(std::false_type{}, t, st);
+    else tile(std::true_type{}, t, st);
     __syncwarp();  // y is in the tile
     if (!SUMMARY) {
       const T* ty = sm.tile[st][0];

@@ -126,3 +126,54 @@ def test_scan_in_chunks_of_any_length_and_type(dtype, T, D, n, slots):
     eps, tiny = torch.finfo(dtype).eps, torch.finfo(dtype).tiny
     assert (np.abs(gf - rf) <= tf + np.abs(rf) * orc.U).all()
     assert (np.abs(gy - ry) <= ty + (np.abs(ry) + ty) * eps / 2 + tiny * eps / 2).all()
+
+
+def _define(i, T, D=None, init=None, dt=None):
+    """The definition in 64 bits, token by token, infinities and NaN and all. A decay below 2^-126 is
+    zero in fp32 arithmetic without subnormal numbers, and zero times an infinite state is NaN:
+    so it is here, where 64 bits would hold the decay (exp(dt A) for dt A < -87.3)."""
+    x, B, C, A = (_n64(i[k]) for k in ("x", "B", "C", "A"))
+    d = orc.softplus(_n64(i["dt"])) if dt is None else dt
+    h = np.zeros(A.shape) if init is None else init.astype(np.float64)
+    ys = []
+    with np.errstate(all="ignore"):
+        for t in range(T):
+            a = np.exp(d[t][:, None] * A)
+            h = np.where(a < 2.0 ** -126, 0.0, a) * h + (d[t] * x[t])[:, None] * B[t]
+            ys.append((C[t] * h).sum(1) + (0.0 if D is None else D * x[t]))
+    return np.stack(ys), h
+
+
+def _alike(got, ref, what=""):
+    """Infinities with their signs, NaN and finite values at the same places."""
+    g = _n64(got)
+    assert np.array_equal(np.isnan(g), np.isnan(ref)), (what, "NaN", np.argwhere(np.isnan(g) != np.isnan(ref))[:4])
+    w = np.isinf(ref) | np.isinf(g)
+    assert np.array_equal(np.where(w, g, 0), np.where(w, ref, 0)), (what, np.argwhere(w)[:4])
+
+
+def _infinities(T, n, dtype, places, skips):
+    from pto_fuser import ssm_scan
+    D = 12
+    for at in {T - 1, T // 2}:
+        for where in places:
+            i = _scan_inputs(T, D, n, dtype, seed=n)
+            for k in ("B", "C"):      # of one sign: an infinite input has an infinite output
+                i[k] = i[k].abs() + 0.25
+            i[where][(at, 0, n - 1) if where in "BC" else (at, 3)] = float("inf")
+            c = {k: v.cuda() for k, v in i.items()}
+            for skip in skips:
+                y, f = ssm_scan(c["x"][None], c["dt"][None], c["A"], c["B"][None], c["C"][None],
+                                D=skip and c[skip])
+                ry, rf = _define(i, T, D=skip and _n64(i[skip]))
+                _alike(f[0], rf, (where, at, skip, "final"))
+                _alike(y[0], ry, (where, at, skip, "y"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [1, 4, 7, 12, 16, 33, 70])
+@pytest.mark.parametrize("T", [1, 16, 21, 40])
+def test_scan_infinite_B_and_C(T, n, dtype):
+    """An infinity in B or C at the last and at an earlier token: outputs and final state are
+    infinite or NaN exactly where the definition is."""
+    _infinities(T, n, dtype, ("B", "C"), (None, "D"))
