@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const 
 #pragma unroll
       for (int off = TL; off < LANES; off *= 2)
         v = add2(v, __shfl_xor_sync(0xffffffffu, v, off));
-      v = fma2(skip, xv, v);
+      if (a.D) v = fma2(skip, xv, v);  // (zero times an infinite x would stay)
       if (zp) v = mul2(v, silu2(zv));
       if (lane < TL) st_pair<T>(tx, v);  // over x, which all have read
     }
@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(kScanStepThreads, LANES < 4 ? 4 : 8) ssm_scan_
       const float xv = to_f32<T>(rx[q]);
       dx[q] = d[q] * xv;
       d[q] *= kLog2e;  // exp(dt' A) = 2^(dt' log2(e) A)
-      sx[q] = skip[q] * xv;
+      sx[q] = a.D ? skip[q] * xv : 0.f;
       gate[q] = a.z ? silu_f32(to_f32<T>(rz[q])) : 1.f;
     }
 #pragma unroll

@@ -177,3 +177,35 @@ def test_scan_infinite_B_and_C(T, n, dtype):
     """An infinity in B or C at the last and at an earlier token: outputs and final state are
     infinite or NaN exactly where the definition is."""
     _infinities(T, n, dtype, ("B", "C"), (None, "D"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [8, 16, 64])
+@pytest.mark.parametrize("T", [1, 16, 21, 40])
+def test_scan_infinite_x_and_dt(T, n, dtype):
+    """The same for x and dt, with a skip and without one (which is not a skip of zero)."""
+    _infinities(T, n, dtype, ("x", "dt"), (None, "D"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,D,n", [(3, 12, 8), (3, 12, 16), (2, 12, 64), (700, 1040, 16)])
+def test_scan_step_infinities(M, D, n, dtype):
+    from pto_fuser import ssm_scan_step
+    for where in ("x", "dt", "B", "C", "state"):
+        i = _scan_inputs(M, D, n, dtype, seed=n)
+        for k in ("B", "C"):
+            i[k] = i[k].abs() + 0.25
+        state = torch.randn(M, D, n, generator=_gen(3))
+        if where == "state":
+            state[1, 3, n - 1] = float("inf")
+        else:
+            i[where][(1, 0, n - 1) if where in "BC" else (1, 3)] = float("inf")
+        c = {k: v.cuda() for k, v in i.items()}
+        for skip in (None, "D"):
+            st = state.cuda()
+            y = ssm_scan_step(c["x"], c["dt"], c["A"], c["B"], c["C"], st, D=skip and c[skip])
+            for m in (0, 1):
+                one = {k: v[m:m + 1] if k in ("x", "dt", "B", "C") else v for k, v in i.items()}
+                ry, rf = _define(one, 1, D=skip and _n64(i[skip]), init=_n64(state[m]))
+                _alike(st[m], rf, (where, m, skip, "state"))
+                _alike(y[m:m + 1], ry, (where, m, skip, "y"))
