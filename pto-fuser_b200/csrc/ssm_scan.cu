@@ -189,7 +189,10 @@ struct ScanSmem {
 // next (softplus, B and C to fp32). x, dt, z, B and C come through shared memory a tile of
 // groups ahead (one asynchronous copy for many tokens, reads at constant offsets), y
 // leaves through the tile of x.
-template <typename T, int LANES, int SPL, int TILE, int G, bool SUMMARY>
+//
+// States with padding (PAD): theirs are zero as B and C are there, unless dt' or dt' x is infinite or
+// NaN. The warp looks for that while it prepares a group and then takes the guarded pass.
+template <typename T, int LANES, int SPL, int TILE, int G, bool SUMMARY, bool PAD>
 __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const ScanArgs a) {
   constexpr int NP = LANES * SPL;            // states with padding
   constexpr int CW = 64 / LANES;             // channels of a warp
@@ -311,6 +314,7 @@ __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const 
   // of this lane's token, B and C as fp32. Steps behind the chunk are zero: they leave the
   // state as it is.
   constexpr int kM = SUMMARY ? 1 : 2, kBC = (TL * NP * kM / 4 + 31) / 32;
+  bool odd = false;  // PAD: the prepared group needs the guarded pass
   auto prepare = [&](int t, int st, int g) {
     const T* tx = &sm.tile[st][0][(g * TL + tok) * CW + 2 * wp];
     Pack<T, 4> raw[kBC];
@@ -327,6 +331,10 @@ __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const 
     both.x = d;
     both.y = mul2(d, xv);
     if (t + TILE > t1 && t + g * TL + tok >= t1) both.x = both.y = pack2(0.f, 0.f);
+    if (PAD) {
+      const float2 zero = unpack2(mul2(add2(both.x, both.y), pack2(0.f, 0.f)));
+      odd = __any_sync(0xffffffffu, !(zero.x == 0.f && zero.y == 0.f));
+    }
     if (SUMMARY && lane < TL) dt_tile = add2(dt_tile, both.x);
     *reinterpret_cast<ulonglong2*>(sm.d[g % 2][tok * (CW / 2) + wp]) = both;
 #pragma unroll
@@ -372,7 +380,10 @@ __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const 
           const float2 u = unpack2(mul2(both.x, A2[k]));
           E[i][k] = pack2(fast_exp2(u.x), fast_exp2(u.y));
           X[i][k] = pack2(dx.x * bv.v[k], dx.y * bv.v[k]);
-          if (guard.value && t + g * TL + i0 + i >= t1) X[i][k] = pack2(0.f, 0.f);
+          if (guard.value) {
+            if (PAD && lane * SPL + k >= a.n) E[i][k] = X[i][k] = pack2(0.f, 0.f);
+            if (t + g * TL + i0 + i >= t1) X[i][k] = pack2(0.f, 0.f);
+          }
         }
       }
 #pragma unroll
@@ -412,7 +423,8 @@ __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const 
     for (int g = 0; g < NG; ++g) {
       if (g == NG - 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncwarp();
-      group(guard, t, st, g);
+      if (PAD && !guard.value && odd) group(std::true_type{}, t, st, g);
+      else group(guard, t, st, g);
     }
   };
   int st = 0;
@@ -521,7 +533,9 @@ constexpr int kScanStepThreads = 128;
 // lanes of a channel share its elementwise work, here over the ITER channels. 512 rows of
 // 8192 channels and 16 states take 115 us, 0.76 of the copy bandwidth; several rows a block
 // through a ring of asynchronous copies took 114.
-template <typename T, int LANES, int ITER, bool VEC>
+// PAD: states that do not fill the lanes. The others' are zero as B and C are there, and are set to
+// it where dt' or dt' x of any channel of the warp is infinite or NaN.
+template <typename T, int LANES, int ITER, bool VEC, bool PAD>
 __global__ void __launch_bounds__(kScanStepThreads, LANES < 4 ? 4 : 8) ssm_scan_step_kernel(const ScanStepArgs a) {
   constexpr int CH = kScanStepThreads / LANES;
   constexpr int TL = LANES < ITER ? LANES : ITER, PF = ITER / TL;
@@ -599,17 +613,19 @@ __global__ void __launch_bounds__(kScanStepThreads, LANES < 4 ? 4 : 8) ssm_scan_
     return;
   }
   for (int r = m;;) {
-    float d[PF], dx[PF], sx[PF], gate[PF], part[ITER];
+    float d[PF], dx[PF], sx[PF], gate[PF], part[ITER], zero = 0.f;
 #pragma unroll
     for (int q = 0; q < PF; ++q) {
       d[q] = to_f32<T>(rd[q]) + bias[q];
       if (a.softplus) d[q] = softplus_f32(d[q]);
       const float xv = to_f32<T>(rx[q]);
       dx[q] = d[q] * xv;
+      if (PAD) zero = fmaf(d[q] + dx[q], 0.f, zero);
       d[q] *= kLog2e;  // exp(dt' A) = 2^(dt' log2(e) A)
       sx[q] = a.D ? skip[q] * xv : 0.f;
       gate[q] = a.z ? silu_f32(to_f32<T>(rz[q])) : 1.f;
     }
+    const bool odd = PAD && __any_sync(0xffffffffu, !(zero == 0.f));
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       if (i && a.dpg != a.Dch) {
@@ -622,6 +638,12 @@ __global__ void __launch_bounds__(kScanStepThreads, LANES < 4 ? 4 : 8) ssm_scan_
       h[i].y = fmaf(fast_exp2(di * A2[i].y), h[i].y, xi * bv[1]);
       h[i].z = fmaf(fast_exp2(di * A2[i].z), h[i].z, xi * bv[2]);
       h[i].w = fmaf(fast_exp2(di * A2[i].w), h[i].w, xi * bv[3]);
+      if (PAD && odd) {
+        if (k0 >= a.n) h[i].x = 0.f;
+        if (k0 + 1 >= a.n) h[i].y = 0.f;
+        if (k0 + 2 >= a.n) h[i].z = 0.f;
+        if (k0 + 3 >= a.n) h[i].w = 0.f;
+      }
       part[i] = cv[0] * h[i].x;
       part[i] = fmaf(cv[1], h[i].y, part[i]);
       part[i] = fmaf(cv[2], h[i].z, part[i]);
@@ -744,8 +766,10 @@ int launch_scan_ls(ScanArgs a, bool split, cudaStream_t st) {
   if (blocks == 0) return PTOF_OK;
   if (blocks > 0x7fffffffLL) return fail(PTOF_EUNSUPPORTED, "ssm_scan: too many blocks");
   const unsigned grid = static_cast<unsigned>(blocks);
-  const auto summary = ssm_scan_kernel<T, LANES, SPL, TILE, G, true>;
-  const auto scan = ssm_scan_kernel<T, LANES, SPL, TILE, G, false>;
+  // (a padded state's value is of no use to a record)
+  const auto summary = ssm_scan_kernel<T, LANES, SPL, TILE, G, true, false>;
+  const auto scan = a.n == LANES * SPL ? ssm_scan_kernel<T, LANES, SPL, TILE, G, false, false>
+                                       : ssm_scan_kernel<T, LANES, SPL, TILE, G, false, true>;
   static_assert(kSmem <= 48 * 1024, "no kernel attribute is set");
   if (split) summary<<<grid, 32, kSmem, st>>>(a);
   scan<<<grid, 32, kSmem, st>>>(a);
@@ -779,8 +803,9 @@ int launch_step_i(ScanStepArgs a, cudaStream_t st) {
   a.bc_vec = a.n % 4 == 0 && (a.B_rs | a.B_gs | a.C_rs | a.C_gs) % 4 == 0 &&
              ((reinterpret_cast<uintptr_t>(a.B) | reinterpret_cast<uintptr_t>(a.C)) %
               (4 * sizeof(T))) == 0;
-  if (vec) ssm_scan_step_kernel<T, LANES, ITER, true><<<grid, kScanStepThreads, 0, st>>>(a);
-  else ssm_scan_step_kernel<T, LANES, ITER, false><<<grid, kScanStepThreads, 0, st>>>(a);
+  if (!vec) ssm_scan_step_kernel<T, LANES, ITER, false, true><<<grid, kScanStepThreads, 0, st>>>(a);
+  else if (a.n < 4 * LANES) ssm_scan_step_kernel<T, LANES, ITER, true, true><<<grid, kScanStepThreads, 0, st>>>(a);
+  else ssm_scan_step_kernel<T, LANES, ITER, true, false><<<grid, kScanStepThreads, 0, st>>>(a);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? PTOF_OK : cuda_fail(e, "ssm_scan_step launch");
 }

@@ -180,15 +180,19 @@ def test_scan_infinite_B_and_C(T, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
-@pytest.mark.parametrize("n", [8, 16, 64])
+@pytest.mark.parametrize("n", [1, 4, 7, 8, 12, 16, 33, 64, 70])
 @pytest.mark.parametrize("T", [1, 16, 21, 40])
 def test_scan_infinite_x_and_dt(T, n, dtype):
-    """The same for x and dt, with a skip and without one (which is not a skip of zero)."""
+    """The same for x and dt, with a skip and without one (which is not a skip of zero), and with
+    states that do not fill the lanes."""
     _infinities(T, n, dtype, ("x", "dt"), (None, "D"))
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("M,D,n", [(3, 12, 8), (3, 12, 16), (2, 12, 64), (700, 1040, 16)])
+@pytest.mark.parametrize("M,D,n", [(3, 12, 8), (3, 12, 16), (2, 12, 64), (700, 1040, 16),
+                                   # states that do not fill the lanes
+                                   (3, 12, 1), (3, 12, 5), (2, 12, 7), (2, 12, 33), (2, 12, 70),
+                                   (700, 1040, 5)])
 def test_scan_step_infinities(M, D, n, dtype):
     from pto_fuser import ssm_scan_step
     for where in ("x", "dt", "B", "C", "state"):
