@@ -124,6 +124,16 @@ __device__ __forceinline__ float log2_rate(float A) {
   return r;
 }
 
+// The state after a chunk: 2^u h + r, of a record r and the decay 2^u over the chunk. Where 2^u is
+// zero or infinite, though no single step's decay was, an infinite h and one of zero stay
+// what they are.
+__device__ __forceinline__ float join(float u, float h, float r) {
+  const float e = fast_exp2(u), v = fmaf(e, h, r);
+  if (v == v) return v;
+  const float p = e * h;
+  return (p == p || !(fabsf(u) <= 3.40282347e38f) ? p : h) + r;
+}
+
 // A warp's tile [TC tokens][CW channels] from or to global memory, in pieces of PIECE elements.
 // Tokens behind the last are read as the last and not written; channels behind the block's
 // are left alone.
@@ -244,10 +254,16 @@ __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const 
     A2[i] = k < a.n ? pack2(log2_rate(a.A[ca * a.n + k]), log2_rate(a.A[cz * a.n + k]))
                     : pack2(0.f, 0.f);
     h[i] = pack2(0.f, 0.f);
-    const float* hp = a.init + static_cast<int64_t>(n) * a.Dch * a.n + k;
-    if (!SUMMARY && a.init && k < a.n) h[i] = pack2(hp[ca * a.n], hp[cz * a.n]);
   }
-  if (!SUMMARY) {
+  auto state_at = [&](const float* p, int k) { return pack2(p[ca * a.n + k], p[cz * a.n + k]); };
+  if (!SUMMARY && a.init) {
+#pragma unroll
+    for (int i = 0; i < SPL; ++i) {
+      const int k = lane * SPL + i;
+      if (k < a.n) h[i] = state_at(a.init + static_cast<int64_t>(n) * a.Dch * a.n, k);
+    }
+  }
+  if (!SUMMARY && j > 0) {
 #pragma unroll 4
     for (int q = slot - j; q < slot; ++q) {  // the chunks before this one
       const int64_t r = static_cast<int64_t>(q) * a.Dch;
@@ -256,9 +272,27 @@ __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const 
       for (int i = 0; i < SPL; ++i) {
         const int k = lane * SPL + i;
         const float2 u = unpack2(mul2(sum, A2[i]));
-        const float* hp = a.ws_h + r * a.n + k;
         if (k < a.n)
-          h[i] = fma2(pack2(fast_exp2(u.x), fast_exp2(u.y)), h[i], pack2(hp[ca * a.n], hp[cz * a.n]));
+          h[i] = fma2(pack2(fast_exp2(u.x), fast_exp2(u.y)), h[i], state_at(a.ws_h + r * a.n, k));
+      }
+    }
+    // A NaN, which stays through the loop, may come from a decay that is zero or infinite only over
+    // a whole chunk: such states are joined again, with a test at each chunk. (The test in the
+    // loop above took 777 x 512 with 64 states from 41 to 54 us.)
+#pragma unroll
+    for (int i = 0; i < SPL; ++i) {
+      const int k = lane * SPL + i;
+      float2 v = unpack2(h[i]);
+      if (k < a.n && !(v.x == v.x && v.y == v.y)) {
+        v = a.init ? unpack2(state_at(a.init + static_cast<int64_t>(n) * a.Dch * a.n, k)) : make_float2(0.f, 0.f);
+#pragma unroll 1
+        for (int q = slot - j; q < slot; ++q) {
+          const int64_t r = static_cast<int64_t>(q) * a.Dch;
+          const float2 u = unpack2(mul2(pack2(a.ws_dt[r + ca], a.ws_dt[r + cz]), A2[i]));
+          const float2 w = unpack2(state_at(a.ws_h + r * a.n, k));
+          v = make_float2(join(u.x, v.x, w.x), join(u.y, v.y, w.y));
+        }
+        h[i] = pack2(v.x, v.y);
       }
     }
   }

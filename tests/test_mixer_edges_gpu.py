@@ -213,3 +213,32 @@ def test_scan_step_infinities(M, D, n, dtype):
                 ry, rf = _define(one, 1, D=skip and _n64(i[skip]), init=_n64(state[m]))
                 _alike(st[m], rf, (where, m, skip, "state"))
                 _alike(y[m:m + 1], ry, (where, m, skip, "y"))
+
+
+@pytest.mark.parametrize("n", [12, 16])
+def test_scan_infinities_between_chunks(n):
+    """An infinite state stays infinite through chunks whose decay is below 2^-126, and a state of
+    zero stays zero through chunks whose growth is beyond the type."""
+    from pto_fuser import ssm_scan
+    T, D = 700, 20
+    assert _slots(1, T, D, n, F32) > 1
+    i = _scan_inputs(T, D, n, F32, seed=1)
+    i["dt"] = i["dt"].abs() + 1
+    i["x"][10, 3] = float("inf")
+    i["B"] = i["B"].abs() + 0.25
+    c = {k: v.cuda() for k, v in i.items()}
+    y, f = ssm_scan(c["x"][None], c["dt"][None], c["A"], c["B"][None], c["C"][None])
+    ry, rf = _define(i, T)
+    assert np.isinf(rf[3]).all()
+    _alike(f[0], rf, "final")
+    _alike(y[0], ry, "y")
+
+    i = _scan_inputs(T, D, n, F32, seed=2)
+    i["x"][:T - 3] = 0
+    d = -_n64(i["dt"].abs() + 1) / 2       # exp(dt A) > 1 with A < 0
+    c = {k: v.cuda() for k, v in i.items()}
+    y, f = ssm_scan(c["x"][None], torch.tensor(d).float().cuda()[None], c["A"], c["B"][None],
+                    c["C"][None], dt_softplus=False)
+    ry, rf = _define(i, T, dt=torch.tensor(d).float().double().numpy())
+    assert (y[0, :T - 3] == 0).all() and np.isfinite(rf).all()
+    assert torch.isfinite(f).all() and torch.isfinite(y).all()
