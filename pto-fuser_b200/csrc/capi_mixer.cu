@@ -122,7 +122,7 @@ int ptof_ssm_scan_exec(const ptof_ssm_scan_params* p, const void* x, const void*
   int rc = validate(p);
   if (rc) return rc;
   const int b = elem_bytes(p->dtype);
-  const bool any = p->T > 0 && p->N > 0;
+  const bool any = p->T > 0 && p->N > 0, fill = p->T > 0 && p->packed && p->zero_fill;
   rc = check_tensors("ssm_scan", {{x, "x", b, any},
                                   {dt, "dt", b, any},
                                   {A, "A", 4, true},
@@ -133,7 +133,7 @@ int ptof_ssm_scan_exec(const ptof_ssm_scan_params* p, const void* x, const void*
                                   {dt_bias, "dt_bias", 4, false},
                                   {cu, "cu_seqlens", 4, p->packed != 0},
                                   {initial, "initial", 4, false},
-                                  {y, "y", b, any},
+                                  {y, "y", b, any || fill},
                                   {final_state, "final_state", 4, false},
                                   {ws, "ws", 16, false}});
   if (rc) return rc;

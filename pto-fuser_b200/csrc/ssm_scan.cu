@@ -721,6 +721,23 @@ __global__ void __launch_bounds__(kScanStepThreads, LANES < 4 ? 4 : 8) ssm_scan_
   }
 }
 
+// Zeros in every token of a packed call without a sequence.
+template <typename T>
+__global__ void __launch_bounds__(256) zero_tokens_kernel(T* y, int64_t ts, int tokens, int D) {
+  const int64_t all = static_cast<int64_t>(tokens) * D, step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < all; i += step)
+    y[i / D * ts + i % D] = from_f32<T>(0.f);
+}
+template <typename T>
+int launch_zero_tokens(void* y, int64_t ts, int tokens, int D, cudaStream_t st) {
+  const int64_t blocks = (static_cast<int64_t>(tokens) * D + 255) / 256;
+  if (blocks == 0) return PTOF_OK;
+  zero_tokens_kernel<T><<<static_cast<unsigned>(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, st>>>(
+      static_cast<T*>(y), ts, tokens, D);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? PTOF_OK : cuda_fail(e, "ssm_scan launch");
+}
+
 // Lanes of a channel pair, states of a lane and the chunk length for a prompt call.
 struct ScanPlan {
   int lanes, spl, S, slots, per_seq;
@@ -873,7 +890,11 @@ int launch_ssm_scan(const ptof_ssm_scan_params& p, const void* x, const void* dt
                     const void* B, const void* C, const float* D, const void* z, const float* bias,
                     const int* cu, const float* init, void* y, float* fin, void* ws,
                     cudaStream_t st) {
-  if (p.N == 0) return PTOF_OK;
+  if (p.N == 0) {
+    if (!p.packed || !p.zero_fill) return PTOF_OK;
+    if (p.dtype == PTOF_F32) return launch_zero_tokens<float>(y, p.y_token_stride, p.T, p.D, st);
+    return launch_zero_tokens<__half>(y, p.y_token_stride, p.T, p.D, st);  // (bf16's zero too)
+  }
   const ScanPlan q = scan_plan(p);
   ScanArgs a{};
   a.x = x; a.dt = dt; a.A = A; a.B = B; a.C = C; a.D = D; a.z = z; a.bias = bias;

@@ -388,14 +388,9 @@ def ssm_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor
         raise _failed(nv.EINVAL)
     outs = ((x.shape, x.dtype), ((N, ch, n), torch.float32))[:1 + bool(output_final_state)]
     final = 1 if output_final_state else _NULL
-    no_sequence = packed and N == 0      # nothing is launched: only y's zeros are left to do
-    r = _launch(call, "ptof_ssm_scan_exec", p,
-                (0, 1, 2, 3, 4, 5, 6, 7, 9, 8, _OUT, _OUT + 1 if output_final_state else _NULL,
-                 _SCRATCH, _SCRATCH_BYTES), outs, (0, final), scratch=need, out=out,
-                keep=not no_sequence)
-    if no_sequence and out is None:
-        r[0].zero_()
-    return r
+    return _launch(call, "ptof_ssm_scan_exec", p,
+                   (0, 1, 2, 3, 4, 5, 6, 7, 9, 8, _OUT, _OUT + 1 if output_final_state else _NULL,
+                    _SCRATCH, _SCRATCH_BYTES), outs, (0, final), scratch=need, out=out)
 
 
 def ssm_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor,

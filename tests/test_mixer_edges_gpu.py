@@ -242,3 +242,22 @@ def test_scan_infinities_between_chunks(n):
     ry, rf = _define(i, T, dt=torch.tensor(d).float().double().numpy())
     assert (y[0, :T - 3] == 0).all() and np.isfinite(rf).all()
     assert torch.isfinite(f).all() and torch.isfinite(y).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_scan_c_entry_without_a_sequence(dtype):
+    """A packed call of no sequence: its tokens get zeros with zero_fill, else stay."""
+    from pto_fuser import native as nv
+    T, D, pitch, n = 37, 20, 23, 16
+    dest = torch.full((T, pitch), 3.0, dtype=dtype, device="cuda")
+    cu = torch.zeros(1, dtype=torch.int32, device="cuda")
+    A = torch.ones(D, n, device="cuda")
+    s = [0, D] * 3 + [0, pitch] + [0, n, 0] * 2
+    for fill in (0, 1):
+        p = nv.SsmScanParams(*s, 0, T, D, n, 1, nv.dtype_code(dtype), 1, 1, fill, 0)
+        y = dest[:, 2:2 + D]
+        nv.check(nv.lib().ptof_ssm_scan_exec(
+            ctypes.byref(p), None, None, nv.ptr(A), None, None, None, None, None, nv.ptr(cu), None,
+            y.data_ptr(), None, None, 0, nv.stream_handle(dest.device)))
+        assert (y == (0.0 if fill else 3.0)).all()
+        assert (dest[:, :2] == 3.0).all() and (dest[:, 2 + D:] == 3.0).all()
