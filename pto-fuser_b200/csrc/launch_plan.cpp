@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -78,6 +79,7 @@ bool signature(PyObject* const* args, Py_ssize_t n, Key& key, const at::Tensor**
     key.v.push_back(x);
   }
   const bool grad = c10::GradMode::is_enabled();
+  const bool tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   count = static_cast<int>(n - 2);
   for (int i = 0; i < count; ++i) {
     PyObject* o = args[i + 2];
@@ -89,7 +91,7 @@ bool signature(PyObject* const* args, Py_ssize_t n, Key& key, const at::Tensor**
     if (!THPVariable_CheckExact(o)) return false;
     const at::Tensor& x = THPVariable_Unpack(o);
     if (x.layout() != at::kStrided || !x.is_cuda() || x.dim() > 8 || (grad && x.requires_grad()) ||
-        x.is_neg() || x.is_conj() || !x.has_storage())
+        x.is_neg() || x.is_conj() || !x.has_storage() || (tangents && x._fw_grad(0).defined()))
       return false;
     t[i] = &x;
     key.v.push_back((static_cast<int64_t>(x.dim()) << 32) |

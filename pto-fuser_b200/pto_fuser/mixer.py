@@ -11,7 +11,7 @@ them, each in its form for prompts and, where it keeps a state, for single token
 Like the chunked forwards they launch on the current CUDA stream of the tensors' device
 without synchronising, can be captured in a CUDA graph, raise ``ValueError`` /
 ``TypeError`` for wrong arguments and ``NativeError`` for a failed launch, and have no
-backward: a call that would have to record one is refused. Scratch comes from torch's
+derivatives: a call that would have to record a backward or carry a tangent is refused. Scratch comes from torch's
 caching allocator, call by call, so calls on several streams and several captured graphs
 never share any. They have no counterpart in the reference package.
 
@@ -32,6 +32,7 @@ import math
 from typing import Dict, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import native as nv
 
@@ -69,6 +70,10 @@ def _no_backward(what: str, *tensors) -> None:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{what} has no backward: call it under torch.no_grad() or on "
                                  "detached tensors")
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{what} has no forward-mode derivative: call it on the primals")
 
 
 def _sizes(what: str, *sizes: int) -> None:

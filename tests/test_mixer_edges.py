@@ -1,0 +1,47 @@
+"""Arguments of the operators around a recurrent mixer that are refused although their shapes and
+types are right, checked before anything touches a device."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import pto_fuser as pf
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def z(*s, dtype=BF16):
+    return torch.zeros(*s, dtype=dtype)
+
+
+def _calls():
+    """Each entry point with its tensors by name."""
+    A, st = z(8, 4, dtype=F32), z(4, 8, 4, dtype=F32)
+    return {
+        pf.short_conv: dict(x=z(2, 5, 8), weight=z(8, 4), bias=z(8), initial_state=z(2, 3, 8)),
+        pf.short_conv_step: dict(x=z(3, 8), state=z(4, 3, 8), weight=z(8, 4), bias=z(8)),
+        pf.ssm_scan: dict(x=z(2, 5, 8), dt=z(2, 5, 8), A=A, B=z(2, 5, 4), C=z(2, 5, 4),
+                          D=z(8, dtype=F32), z=z(2, 5, 8), dt_bias=z(8, dtype=F32),
+                          initial_state=z(2, 8, 4, dtype=F32)),
+        pf.ssm_scan_step: dict(x=z(3, 8), dt=z(3, 8), A=A, B=z(3, 4), C=z(3, 4), state=st,
+                               D=z(8, dtype=F32), z=z(3, 8), dt_bias=z(8, dtype=F32)),
+        pf.add_rms_norm: dict(x=z(3, 8), weight=z(8), residual=z(3, 8)),
+    }
+
+
+CASES = [(f, k) for f, a in _calls().items() for k in a]
+
+
+@pytest.mark.parametrize("fn,name", CASES, ids=[f"{f.__name__}-{k}" for f, k in CASES])
+def test_forward_mode_tangents_are_refused(fn, name):
+    a = _calls()[fn]
+    with forward_ad.dual_level():
+        a[name] = forward_ad.make_dual(a[name], torch.ones_like(a[name]))
+        with pytest.raises(ValueError, match="no forward-mode derivative"):
+            fn(**a)
+        with torch.no_grad(), pytest.raises(ValueError, match="no forward-mode derivative"):
+            fn(**a)         # no_grad stops the backward only
+        with torch.inference_mode(), pytest.raises(ValueError, match="CUDA tensors"):
+            fn(**a)
+    with pytest.raises(ValueError, match="no forward-mode derivative"):
+        torch.func.jvp(lambda t: fn(**dict(a, **{name: t})), (_calls()[fn][name],),
+                       (torch.ones_like(a[name]),))

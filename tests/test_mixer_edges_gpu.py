@@ -261,3 +261,25 @@ def test_scan_c_entry_without_a_sequence(dtype):
             y.data_ptr(), None, None, 0, nv.stream_handle(dest.device)))
         assert (y == (0.0 if fill else 3.0)).all()
         assert (dest[:, :2] == 3.0).all() and (dest[:, 2 + D:] == 3.0).all()
+
+
+# --------------------------------------------------------------------- launch plans ----
+def _step_call(M=5, D=24, n=16):
+    """A single-token call by its tensors, after one that left its plan."""
+    from pto_fuser import ssm_scan_step
+    g = _gen(7)
+    r = lambda *s, dt=BF16: torch.randn(*s, generator=g).to(dt).cuda()
+    a = dict(x=r(M, D), dt=r(M, D), A=-torch.rand(D, n, generator=g).cuda(), B=r(M, n), C=r(M, n),
+             state=r(M, D, n, dt=F32))
+    ssm_scan_step(**dict(a, state=a["state"].clone()))
+    return ssm_scan_step, a
+
+
+def test_a_plan_does_not_drop_tangents():
+    from torch.autograd import forward_ad
+    fn, a = _step_call()
+    for name in a:
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(a[name], torch.ones_like(a[name]))
+            with pytest.raises(ValueError, match="no forward-mode derivative"):
+                fn(**dict(a, **{name: dual}))
