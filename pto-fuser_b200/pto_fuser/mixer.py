@@ -41,7 +41,8 @@ _byref = ctypes.byref
 
 
 def _tensor(name: str, t: torch.Tensor, shape: tuple, dtype, like: torch.Tensor) -> None:
-    """shape, dtype and device of an argument; its innermost dimension is contiguous."""
+    """shape, dtype and device of an argument; its innermost dimension is contiguous and its
+    memory holds its values."""
     if t.shape != shape:
         raise ValueError(f"{name} shape {tuple(t.shape)} != expected {tuple(shape)}")
     if t.dtype != dtype:
@@ -50,6 +51,8 @@ def _tensor(name: str, t: torch.Tensor, shape: tuple, dtype, like: torch.Tensor)
         raise ValueError(f"{name} on {t.device}, expected {like.device}")
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name} must be contiguous in its last dimension")
+    if t.is_neg():
+        raise ValueError(f"{name} is a negated view of other values: pass {name}.resolve_neg()")
 
 
 def _dense(name: str, t: torch.Tensor, shape: tuple, dtype, like: torch.Tensor) -> None:

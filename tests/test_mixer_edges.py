@@ -45,3 +45,15 @@ def test_forward_mode_tangents_are_refused(fn, name):
     with pytest.raises(ValueError, match="no forward-mode derivative"):
         torch.func.jvp(lambda t: fn(**dict(a, **{name: t})), (_calls()[fn][name],),
                        (torch.ones_like(a[name]),))
+
+
+@pytest.mark.parametrize("fn,name", CASES, ids=[f"{f.__name__}-{k}" for f, k in CASES])
+def test_negated_views_are_refused(fn, name):
+    """The memory of such a view holds the values before the sign."""
+    a = _calls()[fn]
+    a[name] = torch._neg_view(a[name])
+    with pytest.raises(ValueError, match=name + ".resolve_neg"):
+        fn(**a)
+    a[name] = a[name].resolve_neg()
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        fn(**a)

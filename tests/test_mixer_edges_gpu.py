@@ -283,3 +283,10 @@ def test_a_plan_does_not_drop_tangents():
             dual = forward_ad.make_dual(a[name], torch.ones_like(a[name]))
             with pytest.raises(ValueError, match="no forward-mode derivative"):
                 fn(**dict(a, **{name: dual}))
+
+
+def test_a_plan_does_not_drop_a_sign():
+    fn, a = _step_call()
+    for name in a:
+        with pytest.raises(ValueError, match=name + ".resolve_neg"):
+            fn(**dict(a, **{name: torch._neg_view(a[name])}))
