@@ -338,7 +338,7 @@ PTOF_API int ptof_seg_fix_exec_view(void* ws, void* o, const void* oa, const flo
  * Single tokens come as M rows. Row m uses state slot slots[m] (device int32 [M];
  * NULL: slot m), updated in place. A row whose slot lies outside [0, slots) is padding:
  * no state is touched and its y is zero. Rows that share a slot are applied in row
- * order. */
+ * order. The state must not overlap another tensor. */
 
 /* y[t, d] = act(bias[d] + sum_j w[d, j] x[t - width + 1 + j, d]); inputs before a
  * sequence come from initial [N, width - 1, D] (oldest first; NULL: zeros), final

@@ -59,6 +59,7 @@ struct Plan {
   int device = 0;
   int results[kMaxOuts];  // output indexes, kNull for None
   int n_results = 0;
+  int writes = kNull;  // index of a tensor that the call updates
 };
 
 // A call holds its plan: making its results can run Python code that leaves other plans.
@@ -103,6 +104,27 @@ bool signature(PyObject* const* args, Py_ssize_t n, Key& key, const at::Tensor**
   return true;
 }
 
+// First and last + 1 byte that a tensor can touch.
+void span(const at::Tensor& t, uintptr_t& a, uintptr_t& b) {
+  a = b = 0;
+  if (t.numel() == 0) return;
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  a = reinterpret_cast<uintptr_t>(t.data_ptr());
+  b = a + static_cast<uintptr_t>(last + 1) * t.element_size();
+}
+// Whether the memory of t[w], as a whole, reaches into another tensor's.
+bool reaches(const at::Tensor* const* t, int count, int w) {
+  uintptr_t a, b, c, d;
+  span(*t[w], a, b);
+  for (int i = 0; i < count; ++i) {
+    if (i == w || !t[i]) continue;
+    span(*t[i], c, d);
+    if (c < b && a < d) return true;
+  }
+  return false;
+}
+
 using F = uintptr_t;
 int invoke(void* fn, const F* a, int n) {  // the entry points take pointers and 64-bit integers only
   switch (n) {
@@ -114,8 +136,8 @@ int invoke(void* fn, const F* a, int n) {  // the entry points take pointers and
   return -1;
 }
 
-// run(op, flags, tensors...) -> None where no plan has the signature, the entry point's
-// non-zero status as an int, or the tuple of results
+// run(op, flags, tensors...) -> None where no plan has the signature or the call has to be checked
+// anew, the entry point's non-zero status as an int, or the tuple of results
 PyObject* run(PyObject*, PyObject* const* args, Py_ssize_t n) {
   try {
     static thread_local Key key;
@@ -129,6 +151,7 @@ PyObject* run(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (it == plans().end()) Py_RETURN_NONE;
     const std::shared_ptr<const Plan> held = it->second;
     const Plan& p = *held;
+    if (p.writes >= 0 && reaches(t, count, p.writes)) Py_RETURN_NONE;
     const c10::cuda::OptionalCUDAGuard guard(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(p.device)));
     const auto on = at::TensorOptions().device(at::kCUDA, static_cast<c10::DeviceIndex>(p.device));
     at::Tensor outs[kMaxOuts], scratch;
@@ -178,7 +201,7 @@ PyObject* run(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
-// add((op, flags, tensors...), fn, params, args, outs, scratch, results): leaves a plan.
+// add((op, flags, tensors...), fn, params, args, outs, scratch, results, writes): leaves a plan.
 // outs: ((sizes, type code), ...) with codes 0 f32, 1 f16, 2 bf16, 3 e4m3.
 PyObject* add(PyObject*, PyObject* py) {
   try {
@@ -187,8 +210,10 @@ PyObject* add(PyObject*, PyObject* py) {
     const char* params;
     Py_ssize_t bytes;
     long long scratch;
-    if (!PyArg_ParseTuple(py, "O!Ky#O!O!LO!", &PyTuple_Type, &call, &fn, &params, &bytes,
-                          &PyTuple_Type, &args, &PyTuple_Type, &outs, &scratch, &PyTuple_Type, &results))
+    int writes;
+    if (!PyArg_ParseTuple(py, "O!Ky#O!O!LO!i", &PyTuple_Type, &call, &fn, &params, &bytes,
+                          &PyTuple_Type, &args, &PyTuple_Type, &outs, &scratch, &PyTuple_Type, &results,
+                          &writes))
       return nullptr;
     Key key;
     const at::Tensor* t[kMaxTensors];
@@ -223,6 +248,7 @@ PyObject* add(PyObject*, PyObject* py) {
     for (Py_ssize_t i = 0; i < nr; ++i) p.results[p.n_results++] = static_cast<int>(PyLong_AsLong(PyTuple_GET_ITEM(results, i)));
     if (PyErr_Occurred()) return nullptr;
     p.scratch = scratch;
+    p.writes = writes >= 0 && writes < count && t[writes] ? writes : kNull;
     for (int i = 0; i < count; ++i)
       if (t[i]) { p.device = t[i]->get_device(); break; }
     if (plans().size() >= kMaxPlans) plans().clear();
@@ -237,7 +263,7 @@ PyObject* add(PyObject*, PyObject* py) {
 PyMethodDef kMethods[] = {
     {"run", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(run)), METH_FASTCALL,
      "run(op, flags, *tensors): launch by plan; None without one, a status, or the results"},
-    {"add", add, METH_VARARGS, "add(call, fn, params, args, outs, scratch, results): leave a plan"},
+    {"add", add, METH_VARARGS, "add(call, fn, params, args, outs, scratch, results, writes): leave a plan"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_launch", "launch plans of checked calls", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

@@ -22,7 +22,8 @@ zeros in a fresh output and are left as they were in ``out``.
 
 Single tokens come as ``[M, ..]`` rows. Row m updates the state slot ``slots[m]`` (int32 [M]
 on the device; slot m without it) in place. A slot outside the state is padding: nothing is
-touched and the row's output is zero. Rows that share a slot are applied in row order.
+touched and the row's output is zero. Rows that share a slot are applied in row order. The
+state shares no memory with the other arguments.
 """
 from __future__ import annotations
 
@@ -119,6 +120,13 @@ def _apart(what: str, out: torch.Tensor, *others) -> None:
     _own_memory(what, "out", out)
 
 
+def _state_apart(what: str, state: torch.Tensor, *inputs) -> None:
+    """``state``, which is written while inputs are read, shares no memory with them."""
+    if any(t is not None and not _disjoint(state, t) for t in inputs):
+        raise ValueError(f"{what}: state must not share memory with an input")
+    _own_memory(what, "state", state)
+
+
 def _own_memory(what: str, name: str, t: torch.Tensor) -> None:
     """No two elements of a tensor that is written lie at one address."""
     if t.is_contiguous():
@@ -158,14 +166,17 @@ def _run(*call):
 
 
 def _launch(call: tuple, name: str, p, args: tuple, outs: tuple, results: tuple, *,
-            scratch: int = 0, out: Optional[torch.Tensor] = None, keep: bool = True) -> tuple:
+            scratch: int = 0, out: Optional[torch.Tensor] = None, keep: bool = True,
+            writes: int = -1) -> tuple:
     """Launch a checked call ``(op, flags, tensors...)`` and, unless it writes into ``out``,
-    keep it as the plan of its signature."""
+    keep it as the plan of its signature. ``writes``: the index of a tensor that it updates (a
+    later call where that one's memory reaches into another's is checked anew)."""
     fn = getattr(nv.lib(), name)
     if out is None and keep:
         addr = ctypes.cast(fn, ctypes.c_void_p).value
         codes = tuple((tuple(shape), _CODES[dt]) for shape, dt in outs)
-        if nv.launcher().add(call, addr, bytes(p), args, codes, scratch, results):
+        if nv.launcher().add(call, addr, bytes(p), args, codes, scratch, results,
+                             writes):
             r = _run(*call)
             if r is not None:
                 return r
@@ -310,12 +321,12 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
         _tensor("out", out, x.shape, x.dtype, x)
         same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
         _apart("short_conv_step", out, None if same else x, state, weight, bias, slots)
-    _own_memory("short_conv_step", "state", state)
+    _state_apart("short_conv_step", state, x, weight, bias, slots)
     _cuda("short_conv_step", x)
     p = nv.ShortConvStepParams(x.stride(0), D if out is None else out.stride(0), state.stride(0),
                                state.stride(1), M, S, D, W, dt, wd, silu)
     return _launch(call, "ptof_short_conv_step_exec", p, (0, 1, 2, 3, 4, _OUT),
-                   ((x.shape, x.dtype),), (0,), out=out)[0]
+                   ((x.shape, x.dtype),), (0,), out=out, writes=1)[0]
 
 
 # --------------------------------------------------------------------------- scan ----
@@ -433,14 +444,14 @@ def ssm_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.T
         one = [t for t in (x, dt, z)
                if t is None or t.data_ptr() != out.data_ptr() or t.stride() != out.stride()]
         _apart("ssm_scan_step", out, *one, A, B, C, state, D, dt_bias, slots)
-    _own_memory("ssm_scan_step", "state", state)
+    _state_apart("ssm_scan_step", state, x, dt, A, B, C, D, z, dt_bias, slots)
     _cuda("ssm_scan_step", x)
     p = nv.SsmScanStepParams(x.stride(0), dt.stride(0), z.stride(0) if z is not None else 0,
                              ch if out is None else out.stride(0), B.stride(0),
                              _group_stride(B, x), C.stride(0), _group_stride(C, x),
                              state.stride(0), M, S, ch, n, G, dtc, bool(dt_softplus))
     return _launch(call, "ptof_ssm_scan_step_exec", p, (0, 1, 2, 3, 4, 6, 7, 8, 9, 5, _OUT),
-                   ((x.shape, x.dtype),), (0,), out=out)[0]
+                   ((x.shape, x.dtype),), (0,), out=out, writes=5)[0]
 
 
 # --------------------------------------------------------------------------- norm ----

@@ -57,3 +57,26 @@ def test_negated_views_are_refused(fn, name):
     a[name] = a[name].resolve_neg()
     with pytest.raises(ValueError, match="CUDA tensors"):
         fn(**a)
+
+
+def test_a_state_that_shares_memory_with_an_input_is_refused():
+    """It is written while other blocks may still read: a race, whatever the order of the rows."""
+    def refused(fn, a, **over):
+        with pytest.raises(ValueError, match="state must not share memory"):
+            fn(**dict(a, **over))
+    a = _calls()[pf.short_conv_step]
+    st = a["state"]
+    refused(pf.short_conv_step, a, x=st[:3, 1])
+    refused(pf.short_conv_step, a, x=st[:3, 2], slots=z(3, dtype=torch.int32))
+    refused(pf.short_conv_step, a, weight=st.view(-1)[:32].view(8, 4))
+    refused(pf.short_conv_step, a, bias=st[3, 2])
+    a = _calls()[pf.ssm_scan_step]
+    refused(pf.ssm_scan_step, a, A=a["state"][1])
+    refused(pf.ssm_scan_step, a, D=a["state"].view(-1)[8:16])
+    f = {k: v.float() for k, v in a.items()}
+    refused(pf.ssm_scan_step, f, x=f["state"][:3, :, 0].contiguous(), z=f["state"][0].view(4, 8)[:3])
+    slots = z(128, dtype=torch.int32)
+    refused(pf.ssm_scan_step, f, slots=slots[:3], state=slots.view(F32).view(4, 8, 4))
+    pool = z(4, 3, 20)           # columns of one pool, side by side, are apart
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        pf.short_conv_step(pool[:3, 0, 8:16], pool[..., :8], z(8, 4))

@@ -290,3 +290,23 @@ def test_a_plan_does_not_drop_a_sign():
     for name in a:
         with pytest.raises(ValueError, match=name + ".resolve_neg"):
             fn(**dict(a, **{name: torch._neg_view(a[name])}))
+
+
+def test_a_plan_does_not_pass_a_state_that_shares_memory():
+    from pto_fuser import short_conv_step, ssm_scan_step
+    fn, a = _step_call()
+    with pytest.raises(ValueError, match="state must not share memory"):
+        fn(**dict(a, A=a["state"][1]))
+    # columns of one pool: beside each other they pass, and give what they give apart
+    M, D = 5, 24
+    pool = torch.randn(M, 3, 3 * D, generator=_gen(1)).to(BF16).cuda()
+    w = torch.randn(D, 4, generator=_gen(2)).to(BF16).cuda()
+    for _ in range(3):
+        x, state = pool[:, 0, D:2 * D], pool[..., :D]
+        alone = state.clone(memory_format=torch.contiguous_format)
+        want = short_conv_step(x.contiguous(), alone, w)
+        rest = pool[..., D:].clone()
+        assert torch.equal(short_conv_step(x, state, w), want)
+        assert torch.equal(state, alone) and torch.equal(pool[..., D:], rest)
+    with pytest.raises(ValueError, match="state must not share memory"):
+        short_conv_step(pool[:, 0, D - 1:2 * D - 1], pool[..., :D], w)
