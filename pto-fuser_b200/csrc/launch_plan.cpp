@@ -171,6 +171,8 @@ PyObject* run(PyObject*, PyObject* const* args, Py_ssize_t n) {
     a[k++] = reinterpret_cast<F>(c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(p.device)).stream());
     const int rc = invoke(p.fn, a, k);
     if (rc != 0) return PyLong_FromLong(rc);
+    // a backward that saved the updated tensor must not use it
+    if (p.writes >= 0 && !t[p.writes]->is_inference()) t[p.writes]->unsafeGetTensorImpl()->bump_version();
     PyObject* r = PyTuple_New(p.n_results);
     if (!r) return nullptr;
     for (int i = 0; i < p.n_results; ++i) {

@@ -191,6 +191,9 @@ def _launch(call: tuple, name: str, p, args: tuple, outs: tuple, results: tuple,
         ptrs = [special[i] if i < 0 else made[i - _OUT].data_ptr() if i >= _OUT
                 else nv.ptr(tensors[i]) for i in args]
         nv.check(fn(_byref(p), *ptrs, nv.stream_handle(dev)))
+    for t in (out, None if writes < 0 else tensors[writes]):
+        if t is not None:
+            torch.autograd.graph.increment_version(t)     # a backward that saved it must not use it
     return tuple(None if i < 0 else made[i] for i in results)
 
 

@@ -310,3 +310,33 @@ def test_a_plan_does_not_pass_a_state_that_shares_memory():
         assert torch.equal(state, alone) and torch.equal(pool[..., D:], rest)
     with pytest.raises(ValueError, match="state must not share memory"):
         short_conv_step(pool[:, 0, D - 1:2 * D - 1], pool[..., :D], w)
+
+
+def test_updates_in_place_are_seen_by_autograd():
+    """A backward that saved a state or an output buffer before a call wrote into it fails, as after
+    any other update in place, and does not use the new values."""
+    from pto_fuser import short_conv, short_conv_step
+    fn, a = _step_call()
+    w4 = torch.ones(a["x"].shape[1], 4, device="cuda", dtype=BF16)
+    out = torch.empty_like(a["x"])
+    calls = [(a["state"], lambda: fn(**a)), (a["state"], lambda: fn(**a, out=out)),
+             (out, lambda: fn(**a, out=out)), (out, lambda: short_conv(a["x"][None], w4, out=out[None]))]
+    for tensor, call in calls:
+        before = tensor._version
+        call()
+        assert tensor._version == before + 1
+    weight = torch.ones(a["state"].shape[2], device="cuda", requires_grad=True)
+    state = a["state"]
+    loss = (state * weight).sum()
+    fn(**a)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():                        # no versions there, and no error
+        state = torch.zeros_like(a["state"])
+        for _ in range(2):
+            fn(**dict(a, state=state))
+            fn(**dict(a, state=state), out=torch.empty_like(a["x"]))
+    conv = torch.zeros(5, 3, 24, device="cuda", dtype=BF16)
+    for k in range(3):
+        short_conv_step(a["x"], conv, w4)
+        assert conv._version == k + 1
