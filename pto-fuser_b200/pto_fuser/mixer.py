@@ -458,7 +458,8 @@ def ssm_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.T
 
 
 # --------------------------------------------------------------------------- norm ----
-_EPS: Dict[float, int] = {}          # each eps seen, by a number of its own
+_EPS: Dict[float, int] = {}          # eps of late, each by a number that no other one gets
+_EPS_MOST = 256
 _EPS_NUMBERS = itertools.count()
 
 
@@ -482,12 +483,16 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     scale fp32 [.., 1] or [.., ceil(D / group_size)] (None without an 8-bit output)."""
     if type(eps) is not float:
         eps = float(eps)             # a tensor's value, not the tensor, belongs to a signature
+    if not eps >= 0.0:
+        raise ValueError(f"add_rms_norm: eps {eps}")
     fp8 = out_dtype is not None and out_dtype != x.dtype
     plain = group_size is None or type(group_size) is int and 0 < group_size <= 128
     flags = -1
     if plain and (not fp8 or out_dtype == torch.float8_e4m3fn):
         number = _EPS.get(eps)
         if number is None:           # two threads take two numbers, one of them stays
+            if len(_EPS) >= _EPS_MOST:
+                _EPS.clear()
             number = _EPS.setdefault(eps, next(_EPS_NUMBERS))
         flags = number << 10 | (group_size or 0) << 1 | fp8
     call = (_NORM, flags, x, weight, residual)
@@ -507,8 +512,6 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
         rt = _weight_dtype("residual", residual, x)
         _tensor("residual", residual, x.shape, rt, x)
         rd = nv.dtype_code(rt)
-    if not eps >= 0.0:
-        raise ValueError(f"add_rms_norm: eps {eps}")
     if fp8 and out_dtype != torch.float8_e4m3fn:
         raise TypeError(f"add_rms_norm: out_dtype {out_dtype}: expected {x.dtype} or "
                         "torch.float8_e4m3fn")

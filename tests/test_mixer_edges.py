@@ -80,3 +80,19 @@ def test_a_state_that_shares_memory_with_an_input_is_refused():
     pool = z(4, 3, 20)           # columns of one pool, side by side, are apart
     with pytest.raises(ValueError, match="CUDA tensors"):
         pf.short_conv_step(pool[:3, 0, 8:16], pool[..., :8], z(8, 4))
+
+
+def test_values_of_eps_are_not_collected():
+    """Values that never come again, and such as are refused, leave nothing that grows."""
+    from pto_fuser import mixer
+    x, w = z(3, 8), z(8)
+    for k in range(3000):
+        with pytest.raises(ValueError, match="CUDA tensors"):
+            pf.add_rms_norm(x, w, eps=1e-6 * (k + 1))
+        with pytest.raises(ValueError, match="eps"):
+            pf.add_rms_norm(x, w, eps=float("nan"))
+        with pytest.raises(ValueError, match="eps"):
+            pf.add_rms_norm(x, w, eps=-1.0 - k)
+    assert len(mixer._EPS) <= 1000
+    numbers = list(mixer._EPS.values())
+    assert len(set(numbers)) == len(numbers)
