@@ -116,12 +116,13 @@ __device__ __forceinline__ f32x2 softplus2(f32x2 v) {
   return fma2(p, e, pack2(fmaxf(w.x, 0.f), fmaxf(w.y, 0.f)));
 }
 
-// Copies of BYTES (4, 8 or 16, both addresses aligned to it) that land without a register.
+// Copies of BYTES (4, 8 or 16, both addresses aligned to it) that land without a register. The
+// clobber keeps reads of what the place held before them, in program order.
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void* smem, const void* gmem) {
   const uint32_t d = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(gmem));
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(gmem), "n"(BYTES));
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(gmem) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(gmem), "n"(BYTES) : "memory");
 }
 
 // Bounds of sequence n of a packed batch, kept inside [0, T] whatever cu holds.
