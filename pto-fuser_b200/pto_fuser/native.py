@@ -155,6 +155,10 @@ def launcher():
         try:
             from ._native import _launch
         except ImportError as e:
+            if os.path.exists(os.path.join(os.path.dirname(LIB_PATH), "_launch.so")):
+                raise RuntimeError("launch module cannot be loaded: _native/_launch.so was built for "
+                                   "another torch or Python (build it anew with "
+                                   f"`make -C pto-fuser_b200/csrc`): {e}") from e
             raise RuntimeError("launch module not built: _native/_launch.so is missing (build it "
                                "with `make -C pto-fuser_b200/csrc`)") from e
         _launcher = _launch

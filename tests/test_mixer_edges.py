@@ -96,3 +96,18 @@ def test_values_of_eps_are_not_collected():
     assert len(mixer._EPS) <= 1000
     numbers = list(mixer._EPS.values())
     assert len(set(numbers)) == len(numbers)
+
+
+def test_a_launch_module_that_cannot_be_loaded_is_not_called_missing(monkeypatch, tmp_path):
+    import sys
+
+    from pto_fuser import _native, native
+    native.launcher()
+    monkeypatch.setattr(native, "_launcher", None)
+    monkeypatch.delattr(_native, "_launch")
+    monkeypatch.setitem(sys.modules, "pto_fuser._native._launch", None)     # its import fails
+    with pytest.raises(RuntimeError, match="built for another torch or Python"):
+        native.launcher()
+    monkeypatch.setattr(native, "LIB_PATH", str(tmp_path / "lib.so"))
+    with pytest.raises(RuntimeError, match="is missing"):
+        native.launcher()
