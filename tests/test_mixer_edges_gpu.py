@@ -340,3 +340,45 @@ def test_updates_in_place_are_seen_by_autograd():
     for k in range(3):
         short_conv_step(a["x"], conv, w4)
         assert conv._version == k + 1
+
+
+# ------------------------------------------------------------------------ streams ----
+def test_a_call_runs_and_allocates_on_the_calling_stream():
+    """The inputs of calls on a side stream are written there, behind work that takes a while, and
+    results are read there, some dropped at once so that their memory is used again: a launch
+    on another stream would read what is not there yet, a block of another stream's pool would
+    be overwritten while it is read."""
+    from pto_fuser import add_rms_norm, ssm_scan
+    M, D, n = 512, 2048, 16
+    g = _gen(0)
+    rounds = 12
+    values = torch.randn(rounds, 2, M, D, generator=g).to(BF16).cuda()
+    w = torch.ones(D, device="cuda", dtype=BF16)
+    A = -torch.rand(D, n, generator=g).cuda() - 0.1
+    bc = torch.randn(2, 1, M, n, generator=g).to(BF16).cuda()
+
+    def call(x):
+        u = add_rms_norm(x, w)[0]
+        y, f = ssm_scan(u[None], u[None], A, bc[0], bc[1])      # in chunks: it takes scratch
+        return y[0], f
+
+    assert _slots(1, M, D, n, BF16) > 1
+    want = [[tuple(t.clone() for t in call(values[k, lane])) for lane in (0, 1)] for k in range(rounds)]
+    lanes = [torch.cuda.current_stream(), torch.cuda.Stream()]
+    xs = [torch.zeros(M, D, device="cuda", dtype=BF16) for _ in lanes]
+    slow = [torch.randn(4096, 4096, device="cuda", dtype=BF16) for _ in lanes]
+    got = [[None, None] for _ in range(rounds)]
+    torch.cuda.synchronize()
+    for k in range(rounds):
+        for lane, stream in enumerate(lanes):
+            with torch.cuda.stream(stream):
+                for _ in range(6):
+                    slow[lane] @ slow[lane]
+                xs[lane].copy_(values[k, lane])
+                y, f = call(xs[lane])
+                got[k][lane] = (y.clone(), f.clone())
+                del y, f
+    torch.cuda.synchronize()
+    for k in range(rounds):
+        for lane in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(got[k][lane], want[k][lane])), (k, lane)
