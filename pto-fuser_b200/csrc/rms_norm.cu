@@ -11,7 +11,7 @@
 // least: one block of 1024 threads took 121 us for 4096 x 16384 bf16, two of 512 take 80.
 //
 // bf16 with a residual, us and share of the copy bandwidth: 16384 x 8192 to e4m3 with a scale
-// for 128 columns 148, 4096 x 16384 80 (1.0). Rows that begin on no 16 bytes:
+// for 128 columns 147, 4096 x 16384 80 (1.0). Rows that begin on no 16 bytes:
 // 3001 x 5003 f16 with an fp32 residual 31 (0.90; 45 element by element). Such rows to e4m3
 // with a scale a group go element by element, bound by instructions: 4096 x 5001 takes 54
 // where 5000 columns take 35.
@@ -53,15 +53,17 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// Quotients rounded once, as the definition has them: products with rounded reciprocals give 59 %
-// of the scales another last bit, and eight of a million codes the neighbouring e4m3 value.
-// With r within a unit in the last place of 1 / s, q = y r is off by two units at most, and
-// adding r times the remainder y - q s of a fused product rounds to y / s (P. Markstein,
-// Computation of elementary functions on the IBM RISC System/6000 processor, 1990), or, with r
-// not correctly rounded, to its neighbour where y / s lies within 2^-22 units of the middle
-// between two values. That is two instructions a value more than the product alone:
-// 16384 x 8192 to e4m3 with a scale for 128 columns takes 148 us, with products 144, with the
-// library's division and reciprocal 158.
+// Codes are those of y / s rounded once, with the scale s that is returned; products with an
+// approximate reciprocal give some of them the neighbouring e4m3 value. (s itself is a product with
+// the rounded 1 / 448, off by one more half unit than the quotient, as torch's division of a tensor
+// on the device by a number is.) With r within a unit in the last place of 1 / s, q = y r is off by
+// two units at most, and adding r times the remainder y - q s of a fused product rounds to y / s
+// (P. Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990),
+// or, with r not correctly rounded, to its neighbour where y / s lies within 2^-22 units of the
+// middle between two values. That is two instructions a value more than the product alone:
+// 16384 x 8192 to e4m3 with a scale for 128 columns takes 147 us, with the product 144, with the
+// library's reciprocal and division 158. 7.4 of a million codes are not those of 64-bit
+// arithmetic (the row's root, rounded), with the product 8.0.
 constexpr float kLargest = 3.40282347e38f;  // largest finite fp32 value
 
 // Scale and quotients of the values whose largest magnitude is amax.
@@ -78,13 +80,10 @@ struct Scale {
   }
 };
 __device__ __forceinline__ Scale scale_of(float amax) {
-  constexpr float r = 1.f / kFp8Max;
-  const bool finite = amax <= kLargest;
-  const float q = amax * r, rest = finite ? fmaf(q, -kFp8Max, amax) : 0.f;
   Scale o;
-  o.s = max_nan(fmaf(rest, r, q), kTinyScale);
+  o.s = max_nan(amax * (1.f / kFp8Max), kTinyScale);
   o.r = fast_rcp(o.s);  // s is a normal number, its reciprocal at most 2^126
-  o.minus_s = finite ? -o.s : 0.f;
+  o.minus_s = o.s <= kLargest ? -o.s : 0.f;
   return o;
 }
 

@@ -27,23 +27,53 @@ def _n64(t):
 @pytest.mark.parametrize("group", [None, 32, 64, 128])
 @pytest.mark.parametrize("dtype,D", [(F32, 4096), (BF16, 8192), (F16, 1032), (F32, 5003), (BF16, 301),
                                      (F32, 9000), (F16, 8191)])
-def test_norm_scales_and_codes_are_ieee_quotients(dtype, D, group):
+def test_norm_codes_are_ieee_quotients(dtype, D, group):
     """Rows of +-1 have the sum of squares D whatever its order, so the values before the 8-bit
-    form are those of the 32-bit call, bit by bit, and scale = amax / 448 and y / scale are
-    quotients rounded once: no tolerance."""
+    form are those of the 32-bit call, bit by bit; the scale is amax times the rounded 1 / 448, and
+    the codes are y / scale rounded once and then to e4m3: no tolerance."""
     from pto_fuser import add_rms_norm
-    for seed in range(6):
+    for seed in range(40):
         g = _gen(seed)
         w = torch.randn(D, generator=g) * torch.exp(2 * torch.randn(D, generator=g))
-        x = torch.randint(0, 2, (3, D), generator=g).mul(2).sub(1).float()
+        x = torch.randint(0, 2, (1, D), generator=g).mul(2).sub(1).float()
         y = add_rms_norm(x.cuda(), w.cuda())[0].cpu()
         q, _, s = add_rms_norm(x.to(dtype).cuda(), w.cuda(), out_dtype=F8, group_size=group)
         size = group or D
-        parts = torch.nn.functional.pad(y, (0, -D % size)).view(3, -1, size)
-        scale = torch.clamp(parts.abs().amax(-1) / 448.0, min=2.0 ** -126)
-        want = (parts / scale[..., None]).view(3, -1)[:, :D].to(F8)
+        parts = torch.nn.functional.pad(y, (0, -D % size)).view(1, -1, size)
+        scale = torch.clamp(parts.abs().amax(-1) * torch.tensor(1 / 448.0), min=2.0 ** -126)
+        want = (parts / scale[..., None]).view(1, -1)[:, :D].to(F8)
         assert torch.equal(s.cpu(), scale)
         assert torch.equal(q.cpu().float(), want.float())
+
+
+@pytest.mark.parametrize("group", [None, 32, 128])
+@pytest.mark.parametrize("off", [0, 1, 2])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_norm_codes_of_values_between_two_codes(dtype, off, group):
+    """Weights within a few units in the last place of the middles between two e4m3 values, times the
+    scale, over rows of +-1, whose root is 1 with eps = 0 (so y is the weight): the codes are those
+    of the quotient, which a product with a reciprocal misses for some. No tolerance."""
+    from pto_fuser import add_rms_norm
+    D = 1024
+    codes = torch.arange(0, 127, dtype=torch.uint8).view(F8).float()      # 0 to 448
+    middles = (codes[1:] + codes[:-1]) / 2
+    size = group or D
+    for seed in range(4):
+        g = _gen(seed)
+        amax = torch.exp(3 * torch.randn(D // size, 1, generator=g))
+        scale = amax * torch.tensor(1 / 448.0)
+        w = middles[torch.randint(0, len(middles), (D // size, size), generator=g)] * scale
+        bits = w.view(torch.int32) + torch.randint(-2, 3, w.shape, generator=g).to(torch.int32)
+        w = bits.view(F32)
+        w[:, :1] = amax
+        want = (w / scale).view(-1).to(F8).float()
+        sign = torch.randint(0, 2, (2, D), generator=g).mul(2).sub(1).float()
+        big = torch.zeros(2, D + 4, dtype=dtype, device="cuda")
+        x = big[:, off:off + D]
+        x.copy_(sign)
+        q, _, s = add_rms_norm(x, w.view(-1).cuda(), eps=0.0, out_dtype=F8, group_size=group)
+        assert torch.equal(s.cpu(), scale.view(1, -1).expand(2, -1))
+        assert torch.equal(q.cpu().float(), want * sign)
 
 
 def test_norm_to_8_bits_of_values_beyond_the_type():
