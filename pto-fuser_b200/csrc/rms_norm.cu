@@ -8,13 +8,16 @@
 // Bound by memory: x and the residual are read once, the sum, y and the scales written once.
 // TPR threads hold a row in registers between the sum of squares and the output; the
 // partial sums meet in shuffles and, above one warp, in shared memory. Two blocks an SM at
-// least: one block of 1024 threads took 121 us for 4096 x 16384 bf16, two of 512 take 80.
+// least, where the registers leave room: one block of 1024 threads took 121 us for 4096 x 16384
+// bf16 where two of 512 took 80. Rows of more than 2048 16-byte vectors take one of 1024 all the
+// same: 4096 x 16384 fp32 177 us, where its bytes need 166.
 //
-// bf16 with a residual, us and share of the copy bandwidth: 16384 x 8192 to e4m3 with a scale
-// for 128 columns 147, 4096 x 16384 80 (1.0). Rows that begin on no 16 bytes:
-// 3001 x 5003 f16 with an fp32 residual 31 (0.90; 45 element by element). Such rows to e4m3
-// with a scale a group go element by element, bound by instructions: 4096 x 5001 takes 54
-// where 5000 columns take 35.
+// With a residual, inputs changing between calls, us (what the bytes need at the copy bandwidth
+// in brackets; some of what is written last is still in L2 when a kernel ends): bf16
+// 16384 x 8192 to e4m3 with a scale for 128 columns 147 (146), 4096 x 16384 84 (83). Rows that
+// begin on no 16 bytes: 3001 x 5003 f16 with an fp32 residual 34 (28), kernel alone 30; 45 element
+// by element. Such rows to e4m3 with a scale a group go element by element, bound by
+// instructions: 4096 x 5001 takes 54 where 5000 columns take 35.
 #include <cuda_fp8.h>
 
 #include "capi_internal.h"

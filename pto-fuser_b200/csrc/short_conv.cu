@@ -302,8 +302,9 @@ struct ConvStepArgs {
 constexpr int kConvStepThreads = 128;
 
 // One row and 128 threads' channels per block; the state is shifted by one in place. Bound by
-// memory for many rows (512 x 12288: bf16 30 us, f32 36, 0.87 of the copy bandwidth) and by
-// its latency for few. Four channels a thread in every type: with 16-byte vectors of 16-bit
+// memory for many rows and by its latency for few. 512 x 12288 takes 29 us in bf16 and 38 in f32
+// (its bytes need 16 and 31), without slots 23 and 33: every block looks through all the slots for
+// rows that share its own, and reads the taps of its channels again. Four channels a thread in every type: with 16-byte vectors of 16-bit
 // types the registers leave room for half the threads, which took 34 us.
 template <typename T, int VEC, int K, int W>
 __global__ void __launch_bounds__(kConvStepThreads) short_conv_step_kernel(const ConvStepArgs a) {

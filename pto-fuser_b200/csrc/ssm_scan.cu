@@ -7,10 +7,10 @@
 // Every (t, d, n) needs one exponential, so the prompt form is bound by the special-function
 // units (16 a clock and SM), not by memory: at n = 16 a token and channel moves 8 bytes
 // (bf16) and takes n + 3 of them with softplus and the gate. Counted so, at 1965 MHz, one
-// sequence of 16384 tokens and 4096 channels needs 274 us (its bytes 83) and takes 740, of
-// which the pass for the records is 40 %; 8 sequences of 2048 tokens and 5120 channels need 343
-// and take 636 in one pass: the units are busy 56 % of the time and issue slots 75 %, what
-// the products, conversions and shared-memory reads of a state take beside them.
+// sequence of 16384 tokens and 4096 channels needs 274 us (its bytes 83) and takes 735, of
+// which the pass for the records is 42 %; 8 sequences of 2048 tokens and 5120 channels need 343
+// and take 637 in one pass: the units (with the conversions that run there) are busy 64 % of the
+// time and 60 % of the issue slots are taken, with 20 % of the warps that an SM could hold.
 //
 // A long axis with few channels is cut into chunks of S tokens. A first launch runs every
 // chunk but the last of a sequence from a zero state and stores its final state and the sum
@@ -747,8 +747,10 @@ struct ScanPlan {
 // up to 16 warps run on an SM at a time, and with w of them a token takes a warp
 // 55 + 45 SPL + 3.75 SPL w (its own latency, and what it waits for the others at the
 // special-function units); a warp starts in about 3000. The two launches of a chunked call take
-// 1.7 times the tokens together, 12000 to start and 100 a chunk to join the records.
-// Measured at n = 16, bf16: one sequence of 16384 tokens and 4096 channels 2.3 ms whole, 0.74
+// 1.7 times the tokens together, 12000 to start and 100 a chunk to join the records. The
+// constants were measured at n = 16 and are used for every n: with n > 16 registers leave room for
+// 12 warps and shared memory for 9 (fp32, n > 32), 8 (16 bits, n > 64) or 5 (fp32, n > 64), which
+// the count does not know. Measured at n = 16, bf16: one sequence of 16384 tokens and 4096 channels 2.3 ms whole, 0.74
 // ms in chunks of 1024, 0.765 of 1856 and 0.87 of 2048 (14 warps an SM); 8 of 2048 tokens
 // and 5120 channels 0.64 ms whole, 0.88 ms in chunks of 1024.
 ScanPlan scan_plan(const ptof_ssm_scan_params& p) {

@@ -380,7 +380,7 @@ def ssm_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor
     type (f16 / bf16 / f32), tokens may be strided. A [D, n], D [D], dt_bias [D] fp32, n up
     to 128. initial_state [N, D, n] fp32 (zeros without it). max_seqlen: an upper bound of
     the packed lengths, used to plan the launch (a wrong one costs time; results differ by rounding).
-    Returns (y, final_state): y like x and the states after each sequence, [N, D, n] fp32
+    A token's decay below 2^-126 is zero. Returns (y, final_state): y like x and the states after each sequence, [N, D, n] fp32
     (None with output_final_state=False). ``out`` receives y."""
     flags = bool(dt_softplus) | bool(output_final_state) << 1 | min(max_seqlen or 0, _INT_MAX) << 2
     call = (_SCAN, flags, x, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens)
@@ -478,7 +478,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     x [.., D] f16 / bf16 / f32; residual like x, in x's type or fp32; weight [D] in x's type
     or fp32. out_dtype None: y in x's type. ``torch.float8_e4m3fn``: y holds y / scale with
     ``scale = max(amax |y| / 448, 2^-126)`` over each row, or over each ``group_size`` (32, 64
-    or 128) columns, the last group of a row possibly shorter.
+    or 128) columns, the last group of a row possibly shorter (the codes are those of the
+    quotient by the scale that is returned, rounded once before it is rounded to 8 bits).
     Returns (y, h, scale): h rounded once to the residual's type (None without a residual),
     scale fp32 [.., 1] or [.., ceil(D / group_size)] (None without an 8-bit output)."""
     if type(eps) is not float:
