@@ -344,6 +344,11 @@ __global__ void __launch_bounds__(32, SPL <= 4 ? 16 : 12) ssm_scan_kernel(const 
     for (int i = wl; i < 4 * TILE * NP; i += 32)
       if (i % NP >= a.n) r[i] = from_f32<T>(0.f);
   }
+  if (PAD && cw < CW) {  // and in the channels behind the last, so that nothing odd is found there
+    T* x = sm.tile[0][0];
+    for (int i = wl; i < 6 * TILE * CW; i += 32)
+      if (i % CW >= cw) x[i] = from_f32<T>(0.f);
+  }
   // What group `g` of the tile at t (in stage st) needs before its recurrence: dt' and dt' x
   // of this lane's token, B and C as fp32. Steps behind the chunk are zero: they leave the
   // state as it is.
